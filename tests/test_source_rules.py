@@ -1,0 +1,33 @@
+"""Rules that every source, script and build file of the tree keeps, read from the text: no GPU is needed and nothing is run."""
+import os
+import re
+
+from __graft_entry__ import ROOT
+
+CODE = (".hip", ".h", ".cpp", ".c", ".py", ".sh", ".jl")
+LEFT_OUT = {".git", "_work", "gpurun_out", "profiles", "docs", "__pycache__", ".pytest_cache", "obj", "build"}
+
+
+def _sources():
+    """(path, text) of every source, script and Makefile of the tree, this file left out."""
+    for d, dirs, files in os.walk(ROOT):
+        dirs[:] = sorted(x for x in dirs if x not in LEFT_OUT)
+        for f in sorted(files):
+            p = os.path.join(d, f)
+            if (f.endswith(CODE) or f == "Makefile") and not os.path.samefile(p, __file__):
+                yield os.path.relpath(p, ROOT), open(p, errors="replace").read()
+
+
+def _places(pattern):
+    rx = re.compile(pattern)
+    return [f"{p}:{i}: {l.strip()}" for p, txt in _sources() for i, l in enumerate(txt.splitlines(), 1) if rx.search(l)]
+
+
+def test_the_walk_sees_the_device_code():
+    seen = {p for p, _ in _sources()}
+    assert {"partitionedarrays.jl_amd/csrc/pa_csr.hip", "partitionedarrays.jl_amd/csrc/Makefile", "tools/probe/spmv_probe.hip", "bench.py"} <= seen
+
+
+def test_no_write_through_the_scalar_data_cache():
+    """The scalar data cache is read-only here: no scalar store or atomic, no write-back or discard of it, comments included."""
+    assert _places(r"\bs_(?:(?:buffer|scratch)_)?(?:store|atomic)_|\bs_dcache_(?:wb|discard)") == []
