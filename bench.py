@@ -117,6 +117,14 @@ class optional_section:
         return True
 
 
+def in_launch_wait_s(env=os.environ):
+    """How long a kernel of an N > 1 run waits for a neighbour before it gives up (PA_IPC_TIMEOUT_S): 10 s, and a fifth of an optional
+    section at most.  A rank lost in a section leaves the others' kernels waiting; a wait has to end, and its launch with it, before
+    the section's timer ends the process: a process must not leave with its kernel still waiting on the GPU."""
+    section = env.get("PA_BENCH_SECTION_TIMEOUT_S")
+    return 10.0 if section is None else min(10.0, float(section) / 5)
+
+
 FP64_VECTOR_PEAK_TFLOPS = 78.6      # MI355X vector fp64 with FMA (256 CUs x 4 SIMDs x 16 lanes x 2 flops x 2.4 GHz); unfused multiply + add: half
 HBM_PEAK_GBPS = 8000.0   # MI355X HBM3E spec peak (MI355X_MICROARCH.md); ~6.3 TB/s is what a copy kernel achieves
 
@@ -927,10 +935,11 @@ def main():
     # stream order and events around the RCCL group (PA_MUL_FUSED=0: round 4's chain, the `north_star` design) -- and rank 0 holds a
     # complete line from then on; the library's default (one launch per part, the exchange waited for INSIDE the launch) is gated and
     # timed behind it as a section that can fail or hang without costing the line.  `value` = the faster of the two that passed its
-    # gate; config.product_path says which.  An in-launch wait gives up after 10 s here (the library's default is 30).
+    # gate; config.product_path says which.  An in-launch wait gives up after 10 s here (the library's default is 30),
+    # sooner where the sections' time is short (in_launch_wait_s).
     want_fused = (N > 1 or world > 1) and os.environ.get("PA_MUL_FUSED", "1") != "0"
     if N > 1 or world > 1:
-        os.environ.setdefault("PA_IPC_TIMEOUT_S", "10")
+        os.environ.setdefault("PA_IPC_TIMEOUT_S", str(in_launch_wait_s()))
         os.environ["PA_MUL_FUSED"] = "0"
     pa = load_package()
     ctx = pa.context()
@@ -1670,7 +1679,6 @@ def main():
     if N > 1 and transport in ("rccl", "host", "torch") and os.environ.get("PA_BENCH_TRANSPORT_AB", "1") != "0":
         with optional_section("transport A/B: ipc push", 120, N, rank):
             import pa_amd.p_vector as pv
-            os.environ.setdefault("PA_IPC_TIMEOUT_S", "5")
             was = pv.TRANSPORT
             pv.TRANSPORT = "ipc"
             try:
