@@ -77,10 +77,9 @@ int pa_ctx_destroy(pa_ctx *ctx);
 int pa_ctx_sync(pa_ctx *ctx);                        /* both streams */
 int pa_ctx_stream(pa_ctx *ctx, int which, void **hip_stream);
 int pa_ctx_device_info(pa_ctx *ctx, int *cus, int *xcds, size_t *hbm_bytes, char *name, size_t name_len);
-/* The comm stream is created with the device's greatest priority (numerically lowest), the compute stream with the
- * least: the pack / RCCL send-recv / unpack kernels of t = consistent!(b) must get CUs while own x own (~300 k
- * workgroups) is running, or the exchange of mul! (src/p_sparse_matrix.jl:2098-2100) is not hidden.  Any out-pointer
- * may be NULL. */
+/* Both streams have the default priority: the pack / RCCL send-recv / unpack kernels of t = consistent!(b) run beside own x own
+ * (src/p_sparse_matrix.jl:2098-2100) in a hardware queue of their own.  least / greatest: the lowest and the highest priority among
+ * the context's two streams (numerically lower = higher).  Any out-pointer may be NULL. */
 int pa_ctx_stream_priority(pa_ctx *ctx, int which, int *priority, int *least, int *greatest);
 
 /* ---- psparse(I,J,V,rows,cols;assembled=true) of one part ON THE DEVICE (csrc/pa_assemble.hip) ------------------------

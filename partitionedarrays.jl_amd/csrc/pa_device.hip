@@ -110,16 +110,11 @@ extern "C" int pa_ctx_create(int device, pa_ctx **out) {
   pa_ctx *c = new pa_ctx();
   c->device = device;
   read_switches(c);
-  // The comm stream gets the highest priority the device offers: own x own puts ~300 k workgroups in front of the
-  // dispatcher, and the pack kernel, RCCL's send/recv kernels and the unpack have to get CUs while it runs or the
-  // exchange does not hide under it (mul!: src/p_sparse_matrix.jl:2098-2100).  Numerically lower = higher priority.
-  int prio_least = 0, prio_greatest = 0;
-  PA_HIP(hipDeviceGetStreamPriorityRange(&prio_least, &prio_greatest));
-  c->comm_priority = prio_greatest;
-  int prio_compute = prio_least;
-  if (const char *e = getenv("PA_COMPUTE_PRIORITY")) prio_compute = atoi(e);     // (measurements)
-  PA_HIP(hipStreamCreateWithPriority(&c->s[0], hipStreamNonBlocking, prio_compute));
-  PA_HIP(hipStreamCreateWithPriority(&c->s[1], hipStreamNonBlocking, prio_greatest));
+  // Two streams of the default priority.  The exchange's kernels get CUs under own x own because they sit in a hardware queue of
+  // their own and own x own's workgroups retire all the time; a raised priority is not used: work on streams of different priorities
+  // has hung this GPU for good.
+  PA_HIP(hipStreamCreateWithFlags(&c->s[0], hipStreamNonBlocking));
+  PA_HIP(hipStreamCreateWithFlags(&c->s[1], hipStreamNonBlocking));
   PA_HIP(hipEventCreateWithFlags(&c->ev_compute, hipEventDisableTiming));
   hipDeviceProp_t prop;
   PA_HIP(hipGetDeviceProperties(&prop, device));
@@ -202,12 +197,11 @@ extern "C" int pa_ctx_stream(pa_ctx *c, int which, void **s) {
 extern "C" int pa_ctx_stream_priority(pa_ctx *c, int which, int *priority, int *least, int *greatest) {
   PA_REQUIRE(c && (which == 0 || which == 1), "bad arguments");
   PA_HIP(hipSetDevice(c->device));
-  int lo = 0, hi = 0, pr = 0;
-  PA_HIP(hipDeviceGetStreamPriorityRange(&lo, &hi));
-  PA_HIP(hipStreamGetPriority(c->s[which], &pr));
-  if (priority) *priority = pr;
-  if (least) *least = lo;
-  if (greatest) *greatest = hi;
+  int pr[2] = {0, 0};
+  for (int k = 0; k < 2; ++k) PA_HIP(hipStreamGetPriority(c->s[k], &pr[k]));
+  if (priority) *priority = pr[which];
+  if (least) *least = std::max(pr[0], pr[1]);
+  if (greatest) *greatest = std::min(pr[0], pr[1]);
   return PA_OK;
 }
 

@@ -87,7 +87,6 @@ struct pa_ctx {
   int64_t n_xalpha[2] = {0, 0};
   bool capturing = false;                 // a pa_graph_begin is open on the compute stream
   bool keep_raw_columns = false;          // pa_ctx_keep_raw_columns: blocks created now keep their Int32 columns in HBM (pa_rowsel.hip)
-  int comm_priority = 0;                  // priority the comm stream was created with (the device's greatest)
   pa_arena *arena = nullptr;              // contiguous HBM extents with their memory-class maps (pa_arena.hip), on demand
   bool arena_tried = false;
   std::mutex mem_mu;                      // guards the arena's maps: create / destroy may come from any host thread

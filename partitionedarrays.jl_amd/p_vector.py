@@ -69,8 +69,7 @@ class Context:
         return Event(self)
 
     def stream_priorities(self):
-        """(compute, comm, least, greatest) stream priorities: the comm stream holds the device's greatest
-        (pa_ctx_stream_priority)."""
+        """(compute, comm, least, greatest) of the context's two streams: the default priority (pa_ctx_stream_priority)."""
         a, b, lo, hi = C.c_int(), C.c_int(), C.c_int(), C.c_int()
         L.call("pa_ctx_stream_priority", self.h, L.STREAM_COMPUTE, C.byref(a), C.byref(lo), C.byref(hi))
         L.call("pa_ctx_stream_priority", self.h, L.STREAM_COMM, C.byref(b), None, None)

@@ -31,3 +31,8 @@ def test_the_walk_sees_the_device_code():
 def test_no_write_through_the_scalar_data_cache():
     """The scalar data cache is read-only here: no scalar store or atomic, no write-back or discard of it, comments included."""
     assert _places(r"\bs_(?:(?:buffer|scratch)_)?(?:store|atomic)_|\bs_dcache_(?:wb|discard)") == []
+
+
+def test_every_stream_has_the_default_priority():
+    """Work on streams of different priorities has hung this GPU for good: nothing asks for another one."""
+    assert _places(r"StreamCreateWithPriority|Stream\([^)]*priority *=|is_high_priority_stream *= *True") == []

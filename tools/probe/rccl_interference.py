@@ -1,5 +1,5 @@
 """what do RCCL's send/recv kernels cost a product kernel that wants all 32 waves per CU?  One rank, one GPU:
-own x own of the 27-point operator (256^3 and 128^3) alone, and with -- per product, queued on the high-priority comm stream
+own x own of the 27-point operator (256^3 and 128^3) alone, and with -- per product, queued on the comm stream
 just before it, as pa_mul5 does -- a 1-rank RCCL group of self-addressed ncclSend / ncclRecv pairs carrying BASELINE config
 4's message set (3 x 65536 + 3 x 256 + 1 doubles: the 7 neighbours of a corner part of (2,2,2) x 256^3), pack kernel
 included.  Third column: the same messages through the push transport's single launch (pa_exchange_push_local on a
