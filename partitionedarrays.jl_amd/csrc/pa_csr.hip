@@ -1611,7 +1611,9 @@ extern "C" int pa_scatter_add(pa_scatter *s, pa_vec *dst, const pa_vec *src, int
   PA_REQUIRE(dst->n_own + dst->n_ghost == s->n_dst && src->n_own + src->n_ghost == s->n_src, "vector sizes do not match the map");
   pa_ctx *c = s->ctx;
   PA_HIP(hipSetDevice(c->device));
-  if (zero_first && s->n_dst) PA_HIP(hipMemsetAsync(dst->d, 0, sizeof(double) * s->n_dst, c->s[0]));
+  // (a kernel, not a memset: this call may be recorded into a graph, and recorded memset nodes have given wrong results on replays)
+  if (zero_first && s->n_dst)
+    hipLaunchKernelGGL(k_fill, dim3(grid_for(s->n_dst, 256)), dim3(256), 0, c->s[0], dst->d, (int64_t)s->n_dst, 0.0);
   if (s->n_tgt)
     hipLaunchKernelGGL(k_unpack_add, dim3((s->n_tgt + 255) / 256), dim3(256), 0, c->s[0], dst->d, src->d, s->d_tgt, s->d_tptr,
                        s->d_tp, (int)s->n_tgt);

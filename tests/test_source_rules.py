@@ -36,3 +36,12 @@ def test_no_write_through_the_scalar_data_cache():
 def test_every_stream_has_the_default_priority():
     """Work on streams of different priorities has hung this GPU for good: nothing asks for another one."""
     assert _places(r"StreamCreateWithPriority|Stream\([^)]*priority *=|is_high_priority_stream *= *True") == []
+
+
+def test_what_a_graph_may_hold_is_cleared_by_a_kernel():
+    """A memset recorded into a graph has given wrong results on replays after the first.  pa_scatter_add is the entry point that
+    clears memory and may be recorded; the library's other memsets stand in calls that create, allocate or synchronise."""
+    txt = dict(_sources())["partitionedarrays.jl_amd/csrc/pa_csr.hip"]
+    body = txt[txt.index('extern "C" int pa_scatter_add('):]
+    body = body[:body.index("\n}")]
+    assert "zero_first" in body and "hipMemset" not in body
