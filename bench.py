@@ -125,6 +125,18 @@ def in_launch_wait_s(env=os.environ):
     return 10.0 if section is None else min(10.0, float(section) / 5)
 
 
+def shared_gpu_env(world, devices):
+    """Switches of ranks that share a GPU (the test mode: never a production run).  PA_FUSED_TAIL_BLOCKS: the fused launch's tail blocks
+    may spin on their neighbours' arrival flags, and eight ranks' worth of spinners must not fill the one GPU the neighbours' pushing
+    blocks have to get onto.  PA_ARENA_FRACTION: a context takes up to 0.70 of the memory it sees free for its extents, as if it had the
+    device to itself; eight ranks of 256^3 rows did hold 248 of 268 GiB, and a rank that came last found none left for its block.  The
+    ranks of a device share that fraction."""
+    devices = max(1, devices)
+    if world <= devices:
+        return {}
+    return {"PA_FUSED_TAIL_BLOCKS": "32", "PA_ARENA_FRACTION": f"{0.70 / -(-world // devices):.4f}"}
+
+
 FP64_VECTOR_PEAK_TFLOPS = 78.6      # MI355X vector fp64 with FMA (256 CUs x 4 SIMDs x 16 lanes x 2 flops x 2.4 GHz); unfused multiply + add: half
 HBM_PEAK_GBPS = 8000.0   # MI355X HBM3E spec peak (MI355X_MICROARCH.md); ~6.3 TB/s is what a copy kernel achieves
 
@@ -903,12 +915,10 @@ def general_csr_entries(pa, ctx, L, host_oo, xv, y_head, n_own, out):
 
 def main():
     args = parse()
-    # ranks sharing a GPU (the test mode: never a production run): the fused launch's tail blocks may spin on their neighbours'
-    # arrival flags, and eight ranks' worth of spinners must not fill the one GPU the neighbours' pushing blocks have to get onto
     try:
         import torch as _t
-        if int(os.environ.get("WORLD_SIZE", "1")) > max(1, _t.cuda.device_count()):
-            os.environ.setdefault("PA_FUSED_TAIL_BLOCKS", "32")
+        for k, v in shared_gpu_env(int(os.environ.get("WORLD_SIZE", "1")), _t.cuda.device_count()).items():
+            os.environ.setdefault(k, v)
     except Exception:                                           # noqa: BLE001
         pass
     N = args.gpus
