@@ -296,7 +296,7 @@ __global__ __launch_bounds__(256) void k_mul_fused(
         if (threadIdx.x == 0) ok = 1;
         __syncthreads();
         for (int i = threadIdx.x; i < n_wait; i += BLK)
-          if (!flag_wait(flags + wait_idx[i], F.seq, ticks)) { atomicExch(F.X->status, 1); ok = 0; }
+          if (!flag_wait(flags + wait_idx[i], F.seq, ticks, F.X->status)) { atomicExch(F.X->status, 1); ok = 0; }
         __syncthreads();
         if (!ok) return;                                     // (a neighbour is gone or out of step: the status word says so)
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "");       // what the neighbours stored in front of their flags is visible now
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(256) void k_mul_fused_pell(const pa_pell_dev P, con
         if (threadIdx.x == 0) ok = 1;
         __syncthreads();
         for (int i = threadIdx.x; i < n_wait; i += BLK)
-          if (!flag_wait(flags + wait_idx[i], F.seq, ticks)) { atomicExch(F.X->status, 1); ok = 0; }
+          if (!flag_wait(flags + wait_idx[i], F.seq, ticks, F.X->status)) { atomicExch(F.X->status, 1); ok = 0; }
         __syncthreads();
         if (!ok) return;
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "");
@@ -572,7 +572,8 @@ int pa_mul_fused_rccl(pa_matrix *m, pa_comm *comm, pa_vec *c, pa_vec *b, double 
   PA_TRY(pa_exchange_pack(p, b, PA_CONSISTENT));
   PA_TRY(pa_exchange_rccl(p, comm, PA_CONSISTENT));
   const unsigned long long seq = ++p->rseq;
-  if (!(cx->sw.test_skip_raise && seq == (unsigned long long)cx->sw.test_skip_raise))
+  const long long skip = cx->sw.test_skip_raise;             // (tests only: this product, or with a minus sign every one from it on)
+  if (!(skip > 0 && seq == (unsigned long long)skip) && !(skip < 0 && seq >= (unsigned long long)-skip))
     hipLaunchKernelGGL(kf_raise, dim3(1), dim3(1), 0, cx->s[1], p->d_rflag, seq);
   PA_HIP(hipGetLastError());
   PA_TRY(pa_mul_fused_launch(m, c, b, alpha, beta, cx->s[0], (const pa_fused_comm *)(p->d_rflag + 2), seq, 0, cx->sw.fused_tail_blocks));

@@ -57,7 +57,7 @@ struct pa_switches {
   int pell = 1;               // PA_SPMV_PELL: blocks that have pattern-ELL storage run on k_spmv_pell (0: the row-split kernel; also read at block creation)
   int pell_bytes = 1;         // PA_SPMV_PELL_BYTES: pattern blocks whose dictionary has 3 .. 64 values run on pattern-ELL's one-byte stream (0: the row-split kernel's; also read at block creation)
   int pell_lean = 1;          // PA_SPMV_PELL_LEAN: slabs of a class run the instruction-lean form (scalar base, lane ballots, scalar bits; pa_pell.h); 0: the masked form everywhere
-  int test_skip_raise = 0;    // PA_TEST_FUSED_SKIP_RAISE=k (tests only): the k-th fused product over RCCL never gets its flag raised -> its tail times out
+  int test_skip_raise = 0;    // PA_TEST_FUSED_SKIP_RAISE=k (tests only): the k-th fused product over RCCL (-k: every one from the k-th on) never gets its flag raised -> its tail times out
   int chain_fused = 1;        // PA_SPMV_CHAIN_FUSED: a column-split chain is built for, and run as, one launch (k_spmv_xring_chain)
 };
 

@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256) void k_push_ipc(const int32_t *__restrict__ id
 __global__ void k_wait_flags(const unsigned long long *__restrict__ flags, const int32_t *__restrict__ which, int n, unsigned long long seq,
                              long long ticks, int *status) {
   for (int i = threadIdx.x; i < n; i += blockDim.x)
-    if (!flag_wait(flags + which[i], seq, ticks)) atomicExch(status, 1);
+    if (!flag_wait(flags + which[i], seq, ticks, status)) atomicExch(status, 1);
 }
 
 __global__ void k_write_flags(unsigned long long *const *__restrict__ dst, int n, unsigned long long seq) {

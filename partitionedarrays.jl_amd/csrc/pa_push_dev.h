@@ -38,8 +38,11 @@ __device__ __forceinline__ unsigned long long flag_load(const unsigned long long
 __device__ __forceinline__ void flag_store(unsigned long long *p, unsigned long long v) {
   __hip_atomic_store(p, v, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
 }
-// spin until *p >= want; false after `ticks` of the 100 MHz wall clock
-__device__ __forceinline__ bool flag_wait(const unsigned long long *p, unsigned long long want, long long ticks) {
+// spin until *p >= want; false after `ticks` of the 100 MHz wall clock, and false as soon as *status says that a wait has given up
+// already: launches queued behind the one that sat out the time-out do not sit it out each in turn (40 queued products took 40
+// time-outs), so that a lost neighbour costs the GPU one time-out, whatever is queued.  The status word (host memory) is read only
+// where the flag is not up yet.
+__device__ __forceinline__ bool flag_wait(const unsigned long long *p, unsigned long long want, long long ticks, const int *status) {
   if (flag_load(p) >= want) return true;
   const long long t0 = (long long)wall_clock64();
   for (;;) {
@@ -47,7 +50,8 @@ __device__ __forceinline__ bool flag_wait(const unsigned long long *p, unsigned 
       if (flag_load(p) >= want) return true;
       __builtin_amdgcn_s_sleep(8);
     }
-    if ((long long)wall_clock64() - t0 > ticks) return false;
+    const int given_up = __hip_atomic_load(status, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    if ((given_up != 0) | ((long long)wall_clock64() - t0 > ticks)) return false;
   }
 }
 
@@ -63,7 +67,7 @@ __device__ __forceinline__ bool pa_push_ipc_block(int *ok, const int32_t *__rest
     int good = 1;
     if (seq > 1 && n > 0) {
       const int sa = push_find_seg(segs, 0, nseg, min(p0, n - 1)), sb = push_find_seg(segs, 0, nseg, min(p0 + 255, n - 1));
-      for (int s = sa; s <= sb && good; ++s) good = flag_wait(segs[s].ack, seq - 1, ticks) ? 1 : 0;
+      for (int s = sa; s <= sb && good; ++s) good = flag_wait(segs[s].ack, seq - 1, ticks, status) ? 1 : 0;
     }
     *ok = good;
   }
