@@ -82,11 +82,14 @@ __device__ __forceinline__ bool pa_push_ipc_block(int *ok, const int32_t *__rest
   __threadfence_system();                              // my stores are in memory before I count myself done
   __syncthreads();
   if (threadIdx.x == 0) {
+    // the counter's top bit: a block of this launch gave up and stored nothing.  Then no slice is announced, whichever block is the
+    // last: a receiver that was only late would take what its buffer still holds for the new values.
+    if (!good) atomicOr(done, 0x80000000u);
     const unsigned t = atomicAdd(done, 1u);
-    if (t == (unsigned)n_blocks - 1) {                 // the last block of the launch announces every slice
+    if ((t & 0x7fffffffu) == (unsigned)n_blocks - 1) { // the last block of the launch announces every slice
       *done = 0;
       __threadfence_system();
-      if (good) for (int s = 0; s < nseg; ++s) flag_store(segs[s].arrive, seq);
+      if ((t >> 31) == 0) for (int s = 0; s < nseg; ++s) flag_store(segs[s].arrive, seq);
     }
   }
   return good;
