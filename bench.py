@@ -125,6 +125,14 @@ def in_launch_wait_s(env=os.environ):
     return 10.0 if section is None else min(10.0, float(section) / 5)
 
 
+def one_launch_section(transport, env=os.environ):
+    """Does the run time mul! as ONE launch, the exchange waited for inside it?  Over the ipc link, whose flags are raised by GPU stores
+    alone.  Over RCCL the wait needs the comm stream's queue to move while a product spins, which no queue owes another: one product
+    after the other, each synchronised, 50 of 50 passed; queued back to back the first timed out and so did all behind it.  There the
+    section would end the run with its time-out, the sections behind it unmeasured: only on request (PA_MUL_FUSED_RCCL=1)."""
+    return transport != "rccl" or env.get("PA_MUL_FUSED_RCCL") == "1"
+
+
 def shared_gpu_env(world, devices):
     """Switches of ranks that share a GPU (the test mode: never a production run).  PA_FUSED_TAIL_BLOCKS: the fused launch's tail blocks
     may spin on their neighbours' arrival flags, and eight ranks' worth of spinners must not fill the one GPU the neighbours' pushing
@@ -1358,10 +1366,9 @@ def main():
     # was faster than the separate launches measured above.  A time-out of an in-launch wait surfaces as an exception from ctx.sync()
     # (the library reports it once and the handle continues on separate launches), a hang ends with the section's timer: either way
     # the line above goes out.
-    if N > 1 and want_fused:
+    if N > 1 and want_fused and one_launch_section(transport):
         with optional_section("fused product", 180, N, rank):
             os.environ.pop("PA_MUL_FUSED", None)
-            os.environ["PA_MUL_FUSED_RCCL"] = "1"        # (over RCCL the one launch is opt-in since round 6: here it is opted into, behind its gate)
             ctx.reload_env()
             ms_sep = ms_per_step
             ok_fused, t_fused, fl0, fl1 = False, None, ctx.fused_launches(), None
@@ -1381,7 +1388,6 @@ def main():
                 use_fused = bool(ok_fused and ms_fused is not None and ms_fused < ms_sep)
                 if not use_fused:                        # the rest of the run stays on the path `value` was measured on
                     os.environ["PA_MUL_FUSED"] = "0"
-                    os.environ.pop("PA_MUL_FUSED_RCCL", None)
                     ctx.reload_env()
             if use_fused:
                 ms_per_step = ms_fused

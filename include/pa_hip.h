@@ -255,7 +255,8 @@ int pa_exchange_rccl(pa_plan *plan, pa_comm *comm, int mode);
  *     replaces pa_exchange_pack + pa_exchange_rccl: the stores travel over xGMI, arrival is a sequence number written behind the
  *     payload, the receiver acknowledges after its unpack (flow control for the next exchange).  A wait that lasts longer than
  *     PA_IPC_TIMEOUT_S (30) raises the link's status (pa_plan_ipc_status: 0 ok, 1 arrival, 2 acknowledgement) and the next
- *     exchange over the link fails with PA_ERR_STATE -- the GPU is never left spinning.  Not inside a graph capture.
+ *     exchange over the link fails with PA_ERR_STATE; exchanges queued behind it give up at once, and of an exchange in which
+ *     an acknowledgement did not come no slice is announced -- the GPU is never left spinning.  Not inside a graph capture.
  * pa_mul5 / pa_mul_no_lat / pa_mul_dot / pa_mul5_transpose with comm == NULL use a connected plan's ipc link. */
 int pa_exchange_push_local(pa_plan *const *plans, int32_t n_parts, pa_vec *const *v, int mode);
 /* pa_exchange_finish of every part behind pa_exchange_push_local in one call (consistent!: one unpack launch for all parts) */

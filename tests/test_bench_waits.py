@@ -44,3 +44,15 @@ def test_the_run_uses_that_wait():
     uses = [m.start() for m in re.finditer("PA_IPC_TIMEOUT_S", code)]
     assert len(uses) == 1
     assert code[uses[0]:].startswith('PA_IPC_TIMEOUT_S", str(in_launch_wait_s()))') and uses[0] < code.index("pa = load_package()")
+
+
+@pytest.mark.parametrize("transport,switch,wanted", [("ipc", None, True), ("ipc", "1", True), ("rccl", None, False), ("rccl", "0", False),
+                                                     ("rccl", "1", True), ("host", None, True)])
+def test_the_wait_inside_the_launch_is_not_timed_over_rccl_unless_asked_for(transport, switch, wanted):
+    env = {} if switch is None else {"PA_MUL_FUSED_RCCL": switch}
+    r = subprocess.run([sys.executable, "-c", f"import bench; print(bench.one_launch_section({transport!r}, {env!r}))"], cwd=ROOT,
+                       capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert r.stdout.split()[-1] == str(wanted)
+    txt = open(os.path.join(ROOT, "bench.py")).read()
+    assert "if N > 1 and want_fused and one_launch_section(transport):" in txt and 'environ["PA_MUL_FUSED_RCCL"]' not in txt
