@@ -5,17 +5,19 @@ import re
 from __graft_entry__ import ROOT
 
 CODE = (".hip", ".h", ".cpp", ".c", ".py", ".sh", ".jl")
-LEFT_OUT = {".git", "_work", "gpurun_out", "profiles", "docs", "__pycache__", ".pytest_cache", "obj", "build"}
+FOLDERS = ("bench", "examples", "include", "oracle", "partitionedarrays.jl_amd", "tests", "tools")
 
 
 def _sources():
-    """(path, text) of every source, script and Makefile of the tree, this file left out."""
-    for d, dirs, files in os.walk(ROOT):
-        dirs[:] = sorted(x for x in dirs if x not in LEFT_OUT)
-        for f in sorted(files):
-            p = os.path.join(d, f)
-            if (f.endswith(CODE) or f == "Makefile") and not os.path.samefile(p, __file__):
-                yield os.path.relpath(p, ROOT), open(p, errors="replace").read()
+    """(path, text) of every source, script and Makefile at the top and in the source folders, this file left out."""
+    paths = [os.path.join(ROOT, f) for f in sorted(os.listdir(ROOT))]
+    for top in FOLDERS:
+        for d, dirs, files in os.walk(os.path.join(ROOT, top)):
+            dirs[:] = sorted(x for x in dirs if x not in ("__pycache__", "obj", "build"))
+            paths += [os.path.join(d, f) for f in sorted(files)]
+    for p in paths:
+        if os.path.isfile(p) and (p.endswith(CODE) or os.path.basename(p) == "Makefile") and not os.path.samefile(p, __file__):
+            yield os.path.relpath(p, ROOT), open(p, errors="replace").read()
 
 
 def _places(pattern):
